@@ -262,7 +262,8 @@ def grouped_desc(a, b, c, offsets=None, groups=1, axis=_ffi.GROUP_ROWS, layout=L
     one group's a.ncols x b.ncols.  ``offsets``: groups + 1 int32 in device memory (an address or a DeviceBuffer), group g has
     rows offsets[g] .. offsets[g + 1]; None: one group of all rows.
 
-    in_type IN_E4M3: ``scale_a`` (ceil(K / 128) x rows) and ``scale_b`` (as b's blocks of 128 x 128 lie) are fp32 in device memory.
+    in_type IN_E4M3: ``scale_a`` (ceil(K / 128) x rows) and ``scale_b`` (as b's blocks of 128 x 128 lie) are fp32 in device memory;
+    ``stride_scale_b``: elements between the groups' scale_b (None: compact, or 0 where the groups share ``b``; 0: all share one).
     Operands given as Matrix, and arrays given as DeviceBuffer, are checked against their buffers (ValueError)."""
     in_bytes, depth = _IN_BYTES.get(in_type, 2), axis == _ffi.GROUP_DEPTH
     c_bytes = 4 if out_type == _ffi.OUT_F32 else 2
@@ -282,7 +283,7 @@ def grouped_desc(a, b, c, offsets=None, groups=1, axis=_ffi.GROUP_ROWS, layout=L
     if scale_a is not None or scale_b is not None:
         k_blocks, across, down = -(-a.ncols // 128), -(-b.ncols // 128), -(-b.nrows // 128)
         if stride_scale_b is None:
-            stride_scale_b = down * (ld_scale_b or across)
+            stride_scale_b = 0 if stride == 0 and not depth else down * (ld_scale_b or across)      # (a shared b has one matrix of scales)
         d.scale_a = _device_array("scale_a", scale_a, (k_blocks - 1) * (ld_scale_a or a.nrows) + a.nrows)
         d.scale_b = _device_array("scale_b", scale_b, (groups - 1) * stride_scale_b + (down - 1) * (ld_scale_b or across) + across)
         d.ld_scale_a, d.ld_scale_b, d.stride_scale_b = ld_scale_a, ld_scale_b, stride_scale_b
