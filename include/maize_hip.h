@@ -331,7 +331,8 @@ typedef struct {
 } maize_gemm_grouped_desc_t;
 int32_t maize_hip_gemm_grouped(maize_ctx_t* ctx, const maize_gemm_grouped_desc_t* desc, void* stream);
 int32_t maize_hip_gemm_grouped_validate(const maize_gemm_grouped_desc_t* desc);
-/* The kernel and grid of a grouped product (the grid covers every table of offsets; workgroups without a tile leave). */
+/* The kernel and grid of a grouped product (the grid covers every table of offsets; workgroups without a tile leave).  A product planned
+ * in K ranges runs without them where its workspace cannot be had: on another tile perhaps, with sums that round in another order. */
 int32_t maize_hip_gemm_grouped_plan(const maize_gemm_grouped_desc_t* desc, uint32_t compute_units, maize_gemm_plan_t* out);
 /* The operands of block-scaled products: x (bf16, half or fp32) -> q (E4M3, same extents) and a scale for every block:
  *   m = max(largest |x| of the block, 2^-100);  scale = m / 448;  q = x * (448 / m), rounded to nearest even

@@ -74,8 +74,8 @@ int32_t maize_hip_gemm_grouped_validate(const maize_gemm_grouped_desc_t* d) {
     return MAIZE_OK;
 }
 
-static int32_t group_planned(const maize_gemm_grouped_desc_t* d, uint32_t cus, maize::GroupPlan* plan) {
-    if (maize::plan_group(*d, cus, plan)) return MAIZE_OK;
+static int32_t group_planned(const maize_gemm_grouped_desc_t* d, uint32_t cus, maize::GroupPlan* plan, bool split = true) {
+    if (maize::plan_group(*d, cus, plan, split)) return MAIZE_OK;
     return report(MAIZE_ERR_SHAPE, "gemm_grouped: more tiles than a launch has workgroups (%u rows, %u groups, N=%u)", d->a.nrows, d->groups, d->c.ncols);
 }
 
@@ -113,7 +113,6 @@ int32_t maize_hip_gemm_grouped(maize_ctx_t* ctx, const maize_gemm_grouped_desc_t
     if (d->groups > 1u) (depth ? args.g.stride_c : args.g.stride_b) = d->stride;
     args.g.batch = 1;
     args.g.layout = d->layout;
-    args.g.ksplit = p.ksplit;
     args.g.lda = d->lda; args.g.ldb = d->ldb; args.g.ldc = d->ldc;
     args.g.alpha = d->alpha; args.g.beta = d->beta;
     args.g.epi = (d->out_type == MAIZE_OUT_F32 ? 1u : 0u) | ((d->alpha != 1.0f || d->beta != 0.0f) ? 2u : 0u) |
@@ -126,7 +125,11 @@ int32_t maize_hip_gemm_grouped(maize_ctx_t* ctx, const maize_gemm_grouped_desc_t
     args.ld_scale_a = d->ld_scale_a ? d->ld_scale_a : d->a.nrows;
     args.ld_scale_b = d->ld_scale_b ? d->ld_scale_b : (d->b.ncols + 127u) / 128u;
     args.stride_scale_b = d->groups > 1u ? d->stride_scale_b : 0u;
-    if (p.workspace_bytes && (rc = maize::stream_workspace(ctx, stream, p.workspace_bytes, &args.g.workspace)) != MAIZE_OK) return rc;
+    // No memory for the K ranges' parts: the same product without K ranges, which needs none.
+    if (p.workspace_bytes && !maize::stream_workspace(ctx, stream, p.workspace_bytes, &args.g.workspace) &&
+        (rc = group_planned(d, maize::compute_units(ctx), &p, false)) != MAIZE_OK)
+        return rc;
+    args.g.ksplit = p.ksplit;
     return maize::launch_more(ctx, p.kernel, p.grid, p.block, stream, &args, sizeof args);
 }
 

@@ -83,7 +83,7 @@ uint32_t group_kernel_count() { return kNameCount; }
 const char* group_kernel_name(uint32_t index) { return index < kNameCount ? kNames[index] : nullptr; }
 const char* quant_kernel_name(uint32_t index) { return index < kQuantKernels ? kQuant[index] : nullptr; }
 
-bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, GroupPlan* out) {
+bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, GroupPlan* out, bool split) {
     const bool bits8 = d.in_type == MAIZE_IN_E4M3, depth = d.axis == MAIZE_GROUP_DEPTH;
     const Shape* shape = shapes(d);
     double best = 0.0;
@@ -94,7 +94,7 @@ bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, Grou
         const uint64_t tiles = most_tiles(d, shape[tile]);
         for (uint32_t ranges : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
             // K ranges: of two K tiles or more; tiles that each have a ticket counter, four rounds (128 x 128: two) of parts at most
-            if (ranges > 1u && (tile == kLarge || k_tiles < 2.0 * ranges || tiles > kTicketBytes / 4u || tiles * ranges > (tile == kFew ? 8u : 4u) * compute_units)) break;
+            if (ranges > 1u && (!split || tile == kLarge || k_tiles < 2.0 * ranges || tiles > kTicketBytes / 4u || tiles * ranges > (tile == kFew ? 8u : 4u) * compute_units)) break;
             const uint64_t items = most_items(d, shape[tile], ranges);
             if (items >= (1u << 24) / (shape[tile].threads / 256u)) break;         // (a launch counts its work items in 32 bits)
             const double cost = estimate(d, tile, ranges, compute_units);

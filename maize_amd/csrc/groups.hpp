@@ -16,8 +16,8 @@ struct GroupPlan {
     uint32_t ksplit;           // K ranges per tile
     size_t workspace_bytes;
 };
-// false: the product needs more workgroups than a launch can have.
-bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, GroupPlan* out);
+// false: the product needs more workgroups than a launch can have.  `split` false: no K ranges, and so no workspace.
+bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, GroupPlan* out, bool split = true);
 
 // Kernel parameter blocks (kernels/gemm_group.hpp, kernels/quantize.hpp).
 struct GroupArgs {

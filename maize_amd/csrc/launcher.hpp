@@ -24,8 +24,9 @@ int add_kernels(const MoreKernels* more);
 __attribute__((format(printf, 2, 3))) int32_t report(int32_t code, const char* fmt, ...);
 
 uint32_t compute_units(const maize_ctx_t* ctx);
-// The stream's scratch memory: as for the split products, zero where a launch leaves it zero.
-int32_t stream_workspace(maize_ctx_t* ctx, void* stream, size_t bytes, void** out);
+// The stream's scratch memory: as for the split products, zero where a launch leaves it zero.  false: it cannot be had (no device memory, or
+// too many are kept for graphs); no error of the runtime is left behind, so that a launch that needs none can follow.
+bool stream_workspace(maize_ctx_t* ctx, void* stream, size_t bytes, void** out);
 // One kernel of the further code object on a grid of `grid` workgroups.
 int32_t launch_more(maize_ctx_t* ctx, uint32_t index, uint32_t grid, uint32_t block, void* stream, const void* args, size_t nbytes);
 

@@ -947,7 +947,11 @@ int32_t report(int32_t code, const char* fmt, ...) {
 
 uint32_t compute_units(const maize_ctx_t* ctx) { return (uint32_t)ctx->prop.multiProcessorCount; }
 
-int32_t stream_workspace(maize_ctx_t* ctx, void* stream, size_t bytes, void** out) { return workspace_for(ctx, stream, bytes, out); }
+bool stream_workspace(maize_ctx_t* ctx, void* stream, size_t bytes, void** out) {
+    if (workspace_for(ctx, stream, bytes, out) == MAIZE_OK) return true;
+    (void)hipGetLastError();
+    return false;
+}
 
 int32_t launch_more(maize_ctx_t* ctx, uint32_t index, uint32_t grid, uint32_t block, void* stream, const void* args, size_t nbytes) {
     if (index >= kMaxMoreKernels || !ctx->more_fn[index]) return fail(MAIZE_ERR_ARG, "launch: kernel %u was not loaded", index);
