@@ -94,27 +94,28 @@ __device__ __forceinline__ u32x4 rsrc_of(uint64_t base, uint32_t bytes) {
 // LDS layout of a K tile of an operand: KC (DIM rows of 128 bytes of K) or rows of K (DIM columns each).
 template <bool KC, uint32_t ES, int DIM>
 struct Tile {
+    static_assert(KC || DIM == 256 || DIM == 128 || (DIM == 64 && ES == 2u), "a layout of maps.hpp (rows of 64 8-bit columns are half lines: no such tile)");
     static constexpr int DEEP = DIM * 64, HALF = DIM * 8;             // rows of K: second half of the tile, second register half
     static __device__ __forceinline__ uint32_t row(uint32_t pc, uint32_t l) {
         if constexpr (KC) return maps::kc_piece_row(pc, l);
-        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_piece_row(pc, l) : DIM == 128 ? maps::sk8n_piece_row(pc, l) : maps::sk8s_piece_row(pc, l);
+        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_piece_row(pc, l) : maps::sk8n_piece_row(pc, l);
         else return DIM == 256 ? maps::sk_piece_row(pc, l) : DIM == 128 ? maps::sk128_piece_row(pc, l) : maps::sk64_piece_row(pc, l);
     }
     static __device__ __forceinline__ uint32_t chunk(uint32_t pc, uint32_t l) {
         if constexpr (KC) return maps::kc_piece_chunk(pc, l);
-        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_piece_chunk(pc, l) : DIM == 128 ? maps::sk8n_piece_chunk(pc, l) : maps::sk8s_piece_chunk(pc, l);
+        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_piece_chunk(pc, l) : maps::sk8n_piece_chunk(pc, l);
         else return DIM == 256 ? maps::sk_piece_chunk(pc, l) : DIM == 128 ? maps::sk128_piece_chunk(pc, l) : maps::sk64_piece_chunk(pc, l);
     }
     // byte offset of chunk `c` (16 bytes) of row `r`
     static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
         if constexpr (KC) return maps::kc_offset(r, c);
-        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_offset(r, c) : DIM == 128 ? maps::sk8n_offset(r, c) : maps::sk8s_offset(r, c);
+        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_offset(r, c) : maps::sk8n_offset(r, c);
         else return DIM == 256 ? maps::sk_offset(r, c) : DIM == 128 ? maps::sk128_offset(r, c) : maps::sk64_offset(r, c);
     }
     // address of the lane's part of fragment `f` (16 rows or columns of the operand), first half; KC: half 1 is at another address
     static __device__ __forceinline__ uint32_t read(uint32_t f, uint32_t half, uint32_t l) {
         if constexpr (KC) return maps::kc_frag16_offset(f * 16u, half, l);
-        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_tr_offset(f, 0, 0, l) : DIM == 128 ? maps::sk8n_tr_offset(f, 0, 0, l) : maps::sk8s_tr_offset(f, 0, 0, l);
+        else if constexpr (ES == 1) return DIM == 256 ? maps::sk8_tr_offset(f, 0, 0, l) : maps::sk8n_tr_offset(f, 0, 0, l);
         else return DIM == 256 ? maps::sk_tr_offset(f, 0, l) : DIM == 128 ? maps::sk128_tr_offset(f, 0, l) : maps::sk64_tr_offset(f, 0, l);
     }
 };
