@@ -93,7 +93,8 @@ bool plan_group(const maize_gemm_grouped_desc_t& d, uint32_t compute_units, Grou
         const double k_tiles = depth ? (double)d.a.nrows / d.groups / 64.0 : (double)cdiv(d.a.ncols, bits8 ? 128u : 64u);
         const uint64_t tiles = most_tiles(d, shape[tile]);
         for (uint32_t ranges : {1u, 2u, 3u, 4u, 6u, 8u, 12u, 16u}) {
-            // K ranges: of two K tiles or more; tiles that each have a ticket counter, four rounds (128 x 128: two) of parts at most
+            // K ranges: of two K tiles or more; tiles that each have a ticket counter; parts for two rounds at most of 128 x 128 (two
+            // workgroups on a compute unit), for 2.7 of 32 x 64 (three) and four of 32 x 128 (two)
             if (ranges > 1u && (!split || tile == kLarge || k_tiles < 2.0 * ranges || tiles > kTicketBytes / 4u || tiles * ranges > (tile == kFew ? 8u : 4u) * compute_units)) break;
             const uint64_t items = most_items(d, shape[tile], ranges);
             if (items >= (1u << 24) / (shape[tile].threads / 256u)) break;         // (a launch counts its work items in 32 bits)
