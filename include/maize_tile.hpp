@@ -126,6 +126,46 @@ inline void gemm_smem_multibuffer(Ctx& ctx, const maize_gemm_ex_desc_t& x, void*
     check(maize_hip_gemm_bf16_ex(ctx.handle(), &x, kernel, stream));
 }
 
+// ---- layers of experts: one product for each group of rows, in one launch ----------------------------
+// Views as above: of the operands' element type, `b` (rows) or `c` (depth) one group's matrix, the groups' matrices behind one
+// another (d.stride; 0: all share one).  What is not an argument is a field of the descriptor: leading dimensions, alpha, beta.
+inline maize_gemm_grouped_desc_t grouped_desc(const Matrix& a, const Matrix& b, const Matrix& c, const int32_t* offsets, uint32_t groups,
+                                              maize_group_axis_t axis = MAIZE_GROUP_ROWS, Layout layout = Layout::NN,
+                                              maize_in_type_t in = MAIZE_IN_BF16, maize_out_type_t out = MAIZE_OUT_SAME) {
+    maize_gemm_grouped_desc_t d{};
+    d.a = a.g.realize(); d.b = b.g.realize(); d.c = c.g.realize();
+    d.offsets = offsets; d.groups = groups;
+    d.axis = axis; d.layout = (uint32_t)layout;
+    const maize_matrix_t& one = axis == MAIZE_GROUP_DEPTH ? d.c : d.b;
+    d.stride = (uint64_t)one.nrows * one.ncols;
+    d.in_type = in; d.out_type = out;
+    d.alpha = 1.0f;
+    return d;
+}
+// The same product of E4M3 operands with block scales, those of the groups' B behind one another (B shared, d.stride == 0: shared).
+inline maize_gemm_grouped_desc_t with_block_scales(maize_gemm_grouped_desc_t d, const float* scale_a, const float* scale_b) {
+    d.in_type = MAIZE_IN_E4M3;
+    d.scale_a = scale_a; d.scale_b = scale_b;
+    d.stride_scale_b = d.stride ? (uint64_t)(d.b.nrows / 128u + (d.b.nrows % 128u ? 1u : 0u)) * (d.b.ncols / 128u + (d.b.ncols % 128u ? 1u : 0u)) : 0u;
+    return d;
+}
+inline maize_gemm_plan_t grouped_plan(const maize_gemm_grouped_desc_t& d, uint32_t compute_units = 256) {
+    maize_gemm_plan_t p;
+    check(maize_hip_gemm_grouped_plan(&d, compute_units, &p));
+    return p;
+}
+inline void gemm_grouped(Ctx& ctx, const maize_gemm_grouped_desc_t& d, void* stream = nullptr) { check(maize_hip_gemm_grouped(ctx.handle(), &d, stream)); }
+
+// x (bf16, half or fp32) to q (E4M3) and a scale for each block of block_rows (1 or 128) x 128: the operands of with_block_scales.
+inline maize_quantize_desc_t quantize_desc(const Matrix& x, const Matrix& q, float* scale, uint32_t block_rows = 1, maize_in_type_t in = MAIZE_IN_BF16) {
+    maize_quantize_desc_t d{};
+    d.x = x.g.realize(); d.q = q.g.realize();
+    d.scale = scale; d.block_rows = block_rows; d.in_type = in;
+    d.batch = 1;
+    return d;
+}
+inline void quantize_blocks(Ctx& ctx, const maize_quantize_desc_t& d, void* stream = nullptr) { check(maize_hip_quantize_blocks(ctx.handle(), &d, stream)); }
+
 // ---- the tile vocabulary ---------------------------------------------------------------------------
 // The reference's caller *traces* its kernel (src/main.rs:31-90): shared-memory ring, Matrix, row / column panels over
 // groups of blocks, sm80_gemm_smem_multibuffer per panel pair.  Here the kernels are hand-written, so the same calls

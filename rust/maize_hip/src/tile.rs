@@ -111,6 +111,14 @@ impl Ctx {
         check(unsafe { ffi::maize_hip_gemm_select(self.h, &d, name.as_mut_ptr(), name.len()) })?;
         Ok(unsafe { CStr::from_ptr(name.as_ptr()) }.to_string_lossy().into_owned())
     }
+    /// Products grouped by expert, or block-scaled ones (`grouped_desc`), on the null stream.
+    pub fn gemm_grouped(&self, d: &ffi::MaizeGemmGroupedDesc) -> Result<()> {
+        check(unsafe { ffi::maize_hip_gemm_grouped(self.h, d, ptr::null_mut()) })
+    }
+    /// Values to E4M3 with a scale for each block (`quantize_desc`), on the null stream.
+    pub fn quantize_blocks(&self, d: &ffi::MaizeQuantizeDesc) -> Result<()> {
+        check(unsafe { ffi::maize_hip_quantize_blocks(self.h, d, ptr::null_mut()) })
+    }
 }
 impl Drop for Ctx {
     fn drop(&mut self) {
@@ -128,6 +136,73 @@ pub fn gemm_desc(a: GlobalMatrix<BF16>, b: GlobalMatrix<BF16>, c: GlobalMatrix<B
         stride_a: 0,
         stride_b: 0,
         stride_c: 0,
+    }
+}
+
+/// What the groups of a grouped product are made of.
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum GroupAxis {
+    /// Rows of A and C; each group has its own B.
+    Rows,
+    /// Rows of A and B; each group has its own C = A^T . B.
+    Depth,
+}
+
+/// One product for each group of rows, groups given by `groups + 1` row numbers in device memory (null with one group: all rows).
+/// `b` (rows) or `c` (depth) is one group's matrix, the groups' matrices lie behind one another; what is not an argument is a field.
+#[allow(clippy::too_many_arguments)]
+pub fn grouped_desc<T, U>(a: GlobalMatrix<T>, b: GlobalMatrix<T>, c: GlobalMatrix<U>, offsets: *const i32, groups: u32, axis: GroupAxis, layout: Layout,
+                          in_type: u32, out_type: u32) -> ffi::MaizeGemmGroupedDesc {
+    let stride = if axis == GroupAxis::Depth { c.nrows as u64 * c.ncols as u64 } else { b.nrows as u64 * b.ncols as u64 };
+    ffi::MaizeGemmGroupedDesc {
+        a: a.raw(),
+        b: b.raw(),
+        c: c.raw(),
+        offsets,
+        groups,
+        axis: if axis == GroupAxis::Depth { ffi::MAIZE_GROUP_DEPTH } else { ffi::MAIZE_GROUP_ROWS },
+        stride,
+        layout: if layout == Layout::NN { ffi::MAIZE_LAYOUT_NN } else { ffi::MAIZE_LAYOUT_NT },
+        lda: 0,
+        ldb: 0,
+        ldc: 0,
+        in_type,
+        out_type,
+        alpha: 1.0,
+        beta: 0.0,
+        scale_a: ptr::null(),
+        scale_b: ptr::null(),
+        ld_scale_a: 0,
+        ld_scale_b: 0,
+        stride_scale_b: 0,
+    }
+}
+
+/// The same product of E4M3 operands with block scales, those of the groups' B behind one another (B shared, stride 0: shared).
+pub fn with_block_scales(mut d: ffi::MaizeGemmGroupedDesc, scale_a: *const f32, scale_b: *const f32) -> ffi::MaizeGemmGroupedDesc {
+    let blocks = |extent: u32| (extent / 128 + u32::from(extent % 128 != 0)) as u64;
+    d.in_type = ffi::MAIZE_IN_E4M3;
+    d.scale_a = scale_a;
+    d.scale_b = scale_b;
+    d.stride_scale_b = if d.stride == 0 { 0 } else { blocks(d.b.nrows) * blocks(d.b.ncols) };
+    d
+}
+
+/// `x` (bf16, half or fp32) to `q` (E4M3) and a scale for each block of `block_rows` (1 or 128) x 128.
+pub fn quantize_desc<T>(x: GlobalMatrix<T>, q: GlobalMatrix<u8>, scale: *mut f32, block_rows: u32, in_type: u32) -> ffi::MaizeQuantizeDesc {
+    ffi::MaizeQuantizeDesc {
+        x: x.raw(),
+        q: q.raw(),
+        scale,
+        block_rows,
+        in_type,
+        ldx: 0,
+        ldq: 0,
+        ld_scale: 0,
+        batch: 1,
+        stride_x: 0,
+        stride_q: 0,
+        stride_scale: 0,
     }
 }
 
